@@ -56,24 +56,31 @@ struct Row {
   __device__ int32_t extra_index(int32_t i) const { return i < head ? i : vocab - extra + i; }
 };
 
-// y(x) = log2(e) (x - m) / T for a reference m >= x (not -inf), one fused multiply-add per logit:
-// with c = log2(e) / T and M = m c rounded, fma(x, c, -M) is (x - m) c but for its own last
-// rounding and that of M, which is the same for every x and taken out of sums by `rest`.
-// Where m c nears the type's range (rows of the type's lowest value) the next lower logit is
-// already so far below that 2^y is 0: any factor that leaves m c in range, exact, and the
-// others far below 0 gives the same 2^y, so a power of two is taken.
+// y(x) = log2(e) (x - m) / T for a reference m >= x (not -inf).
+// Near 0, one fused multiply-add per logit: with c = log2(e) / T and M = m c rounded, fma(x, c, -M)
+// is (x - m) c but for its own last rounding and that of M, which is the same for every x and taken
+// out of sums by `rest`, at most 1/8.  From |m| c = 2^22 on (rows masked by a finite value, very low
+// temperatures) M's rounding would reach whole powers of two: there x - m is taken first, exact
+// for the x near m that count, and nothing is left to take out.
 struct Scale {
-  float c, M, rest;  // 2^y is exp((x - m) / T) 2^rest
-  __device__ Scale(float m, float factor) : c(factor), M(m * factor) {
-    rest = fmaf(m, c, -M);
-    if (is_big(m, factor)) {
-      c = __uint_as_float((364 - ((__float_as_uint(m) >> 23) & 255)) << 23);  // |m| c in [2^110, 2^111)
-      M = m * c;
-      rest = 0.f;
+  float c, off, M, rest;  // 2^y is exp((x - m) / T) 2^rest
+  __device__ Scale(float m, float factor) : c(factor) {
+    const bool far = !(fabsf(m) * factor < 4194304.f);
+    off = far ? m : 0.f;
+    M = far ? 0.f : m * factor;
+    rest = far ? 0.f : fmaf(m, factor, -M);
+  }
+  __device__ float operator()(float x) const { return past_off(x - off); }
+  __device__ float past_off(float x) const { return fmaf(x, c, -M); }  // of x - off
+  // Calls f with a function from logits to their y: without the offset where it is 0, as almost always.
+  template <typename F>
+  __device__ __forceinline__ void with(F f) const {
+    if (off == 0.f) {
+      f([*this](float x) { return past_off(x); });
+    } else {
+      f([*this](float x) { return (*this)(x); });
     }
   }
-  __device__ static bool is_big(float m, float factor) { return fabsf(m) * factor > 1e30f; }
-  __device__ float operator()(float x) const { return fmaf(x, c, -M); }
 };
 
 // Running maximum m, s = sum 2^y and t = sum 2^y y over the logits so far, in 32 bits.
@@ -82,22 +89,19 @@ struct Stats {
   float m, s, t;
 
   __device__ static Stats none() { return {-INFINITY, 0.f, 0.f}; }
-  // Moves the maximum to nm >= m.
-  __device__ void raise(float nm, float c) {
-#pragma clang fp contract(off)
-    if (nm > m) {
-      // between the two scales' M, each rounded: fused, one of the roundings would be missing
-      const float delta = nm * c - m * c;
-      const float r = Scale::is_big(m, c) || Scale::is_big(nm, c) ? 0.f : __builtin_amdgcn_exp2f(-delta);
-      t = r == 0.f ? 0.f : r * (t - delta * s);
-      s *= r;  // 0 * NaN stays NaN
-      m = nm;
-    }
+  // Moves the maximum to nm > m and the sums from scale to scale.
+  __device__ void raise(float nm, const Scale& from, const Scale& to) {
+    const float delta = fmaf(to.off - from.off, to.c, to.M - from.M);  // rests and all
+    const float r = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-delta);
+    t = r == 0.f ? 0.f : r * (t - delta * s);
+    s *= r;  // 0 * NaN stays NaN
+    m = nm;
   }
   // Over a wave, or the first N lanes of every N; every lane gets the same bits.
   template <int N>
   __device__ void join_lanes(float c) {
-    raise(lanes_max<N>(m), c);
+    const float most = lanes_max<N>(m);
+    if (most > m) raise(most, Scale(m, c), Scale(most, c));
     s = lanes_sum<N>(s);
     t = lanes_sum<N>(t);
   }
@@ -115,19 +119,28 @@ struct Stats {
 struct Running : Stats {
   float factor;
   Scale scale;
-  __device__ explicit Running(float c) : Stats(Stats::none()), factor(c), scale(0.f, c) {}
+  bool far = false;  // whether a lane of the wave has a scale with an offset
+  __device__ explicit Running(float c) : Stats(Stats::none()), factor(c), scale(0.f, c) {}  // 2^y of -inf is 0
   template <int N, bool kEnt>
-  __device__ __forceinline__ void absorb(const float (&x)[N], float top) {
+  __device__ __forceinline__ void absorb(float (&x)[N], float top) {
     if (__ballot(top > m) != 0) {
-      raise(fmaxf(m, top), factor);
-      scale = Scale(m == -INFINITY ? 0.f : m, factor);
+      if (top > m) {
+        const Scale to(top, factor);
+        raise(top, scale, to);
+        scale = to;
+      }
+      far = __ballot(scale.off != 0.f) != 0;
+    }
+    if (far) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] -= scale.off;
     }
     // Summed apart first: small terms one by one into a sum that has met the maximum lose more (rows
     // of 200000 fp32, temperature 0.7: gradients 8.7e-7 off those in 64 bits, so 1.2e-7; no slower).
     float near_s = 0.f, near_t = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float y = scale(x[i]);
+      const float y = scale.past_off(x[i]);
       const float e = __builtin_amdgcn_exp2f(y);
       near_s += e;
       if constexpr (kEnt) near_t = fmaf(e, fmaxf(y, -FLT_MAX), near_t);  // -inf adds 0, not 0 * inf
@@ -338,11 +351,12 @@ __device__ __forceinline__ void row_pass(const Row<T>& row, int32_t v0, int32_t 
   if (ends && threadIdx.x < kWave) {  // at most 14 elements, by the first wave, out of order
     const bool in = static_cast<int32_t>(threadIdx.x) < row.extra;
     const int32_t i = in ? row.extra_index(threadIdx.x) : 0;
-    const float x[1] = {in ? to_f32<T>(row.p[i]) : -INFINITY};
-    st.absorb<1, kEnt>(x, x[0]);
+    const float logit = in ? to_f32<T>(row.p[i]) : -INFINITY;
+    float x[1] = {logit};
+    st.absorb<1, kEnt>(x, logit);
     if constexpr (kTop) {
       top.limit(false);
-      if (in) top.add(x[0], i);
+      if (in) top.add(logit, i);
     }
   }
   if constexpr (kTop) top.settle(1);
@@ -604,7 +618,7 @@ __device__ __forceinline__ void map_row(const Row<T>& row, typename T::raw* out,
 template <int kSize, typename T, typename F>
 __device__ __forceinline__ void map_logits(const Row<T>& row, typename T::raw* out, const Range<T>& range,
                                            const Scale& scale, F f) {
-  map_row<kSize>(row, out, range, [&](float x) { return f(scale(x)); });
+  scale.with([&](auto y) { map_row<kSize>(row, out, range, [&](float x) { return f(y(x)); }); });
 }
 
 template <int kSize, typename T>
@@ -951,16 +965,18 @@ __global__ __launch_bounds__(kSize) void distill_step_kernel(DistillParams p, in
   const Scale scale(m, p.c);
   const float a = wt * total / st.s;  // s is of the same scale
   auto f = [&](float y) { return a * __builtin_amdgcn_exp2f(y); };
+  scale.with([&](auto y) {
 #pragma unroll
-  for (int r = 0; r < kHeld; ++r) {
-    const int32_t v = r * kSize + static_cast<int32_t>(threadIdx.x);
-    float x[E];
-    reread(w[r]);
-    unpack<T>(w[r], x);
+    for (int r = 0; r < kHeld; ++r) {
+      const int32_t v = r * kSize + static_cast<int32_t>(threadIdx.x);
+      float x[E];
+      reread(w[r]);
+      unpack<T>(w[r], x);
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = f(scale(x[e]));
-    if (v < row.nvec) store16_once(out + row.index(v), pack<T>(x));
-  }
+      for (int e = 0; e < E; ++e) x[e] = f(y(x[e]));
+      if (v < row.nvec) store16_once(out + row.index(v), pack<T>(x));
+    }
+  });
   range.v0 = held;
   map_logits<kSize>(row, out, range, scale, f);
   terms.write<kSize>(row, out, range, 0, p.top, scale, f);  // `held` is a multiple of kSize, or the whole row
