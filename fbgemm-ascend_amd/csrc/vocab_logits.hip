@@ -904,8 +904,13 @@ __global__ __launch_bounds__(kThreads) void distill_grad_kernel(DistillParams p,
   const Entry t = teacher_entry(p, load_entry(p, row, i), sh);
   const float wt = weight * p.t;
   terms.set(t.q != 0.f ? t.id : -1, -wt * t.q, t.x, p.top);
+  const float total = group_sum(t.q, sh);
+  if (total == 0.f) {  // nothing to learn, also from a row that is no numbers
+    zero_row<kThreads>(row, out, range);
+    return;
+  }
   const Scale scale(m, p.c);
-  const float a = grad_factor(wt * group_sum(t.q, sh), scale, s);
+  const float a = grad_factor(wt * total, scale, s);
   auto f = [&](float y) { return a * __builtin_amdgcn_exp2f(y); };
   map_logits<kThreads>(row, out, range, scale, f);
   terms.write<kThreads>(row, out, range, range.v0, p.top, scale, f);
@@ -958,7 +963,7 @@ __global__ __launch_bounds__(kSize) void distill_step_kernel(DistillParams p, in
   float loss = loss_term(t, st, log_s, p.inv_t), total = t.q;
   group_sum(loss, total, sh);
   store_row(p, i, weight * (p.t * (p.t * loss)), m, st.sum(p.c));
-  if (st.empty()) {
+  if (st.empty() || total == 0.f) {  // no student or no teacher
     zero_row<kSize>(row, out, range);
     return;
   }
