@@ -16,6 +16,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _ext
@@ -24,6 +25,9 @@ _NO_PADDING = -1
 
 
 def _tracks(x: torch.Tensor) -> bool:
+    """Whether the call goes through autograd, which refuses a tangent: there is no forward-mode rule."""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        return True
     return x.requires_grad and torch.is_grad_enabled()
 
 
