@@ -158,8 +158,9 @@ __device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
          lane_xor<J>(static_cast<uint32_t>(v));
 }
 
-// Orders the LDS accesses of one wave (its instructions run in order; this stops the compiler).
-__device__ __forceinline__ void wave_lds_fence() {
+// Orders the accesses of one wave to LDS and memory, of all its lanes (its instructions run in
+// order; this stops the compiler).
+__device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }

@@ -389,9 +389,9 @@ __device__ __forceinline__ uint32_t rank_of(uint32_t digit, bool in, C* count) {
   }
   const int before = __popcll(same & ((1ull << lane_id()) - 1));
   const uint32_t rank = count[digit] + before;
-  wave_lds_fence();
+  wave_fence();
   if (in && before == 0) count[digit] += __popcll(same);
-  wave_lds_fence();
+  wave_fence();
   return rank;
 }
 

@@ -239,7 +239,7 @@ struct TopK {
       atomicMax(kth, at);
       __hip_atomic_store(&shares[threadIdx.x / kWave], part, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
-    wave_lds_fence();
+    wave_fence();
   }
   // Keys [from, to) of the buffer, at most 64, into the list.
   __device__ void merge(int from, int to) {
@@ -251,7 +251,7 @@ struct TopK {
     sort_rising(v);
     list = merge_lists(list, v);
     if (lane_id() == 0) atomicMax(kth, own());
-    wave_lds_fence();
+    wave_fence();
   }
   // This lane's logit x at idx; the lanes of a wave call it apart.  At most 8 times, then settle().
   __device__ void add(float x, uint32_t idx) {
@@ -259,7 +259,7 @@ struct TopK {
     buf[atomicAdd(counter, 1u)] = uint2{__float_as_uint(x), idx};
   }
   __device__ void settle(int most) {
-    wave_lds_fence();
+    wave_fence();
     int count = __builtin_amdgcn_readfirstlane(static_cast<int>(*counter));
     if (count < most) return;
     do {
@@ -268,7 +268,7 @@ struct TopK {
       count = from;
     } while (count >= most);
     if (lane_id() == 0) *counter = count;
-    wave_lds_fence();
+    wave_fence();
     limit(false);
   }
 };
@@ -628,8 +628,8 @@ __device__ __forceinline__ void zero_row(const Row<T>& row, typename T::raw* out
 }
 
 // Tokens of a row whose gradient has a term of its own: out = f(y) + the sum of the token's terms,
-// in the order of the list.  Written after map_logits by the wave that wrote the token's vector:
-// one wave's stores to an address keep their order.
+// in the order of the list.  Written after map_logits by the wave that wrote the token's vector,
+// past a fence of that wave, so that the term is what stays.
 struct Terms {
   int32_t ids[kListed];  // -1: none, or an earlier entry has it
   float sums[kListed], xs[kListed];
@@ -641,7 +641,7 @@ struct Terms {
     const int32_t at = static_cast<int32_t>(threadIdx.x), padded = (n + kAtOnce - 1) / kAtOnce * kAtOnce;
     auto written = [n] {
       if (n <= kWave) {
-        wave_lds_fence();
+        wave_fence();
       } else {
         __syncthreads();
       }
@@ -680,6 +680,7 @@ struct Terms {
   template <int kSize, typename T, typename F>
   __device__ void write(const Row<T>& row, typename T::raw* out, const Range<T>& range, int32_t origin, int32_t n,
                         const Scale& scale, F f) const {
+    wave_fence();
     for (int32_t k = lane_id(); k < n; k += kWave) {
       const int32_t id = ids[k];
       if (id < 0 || !range.holds(row, id)) continue;
