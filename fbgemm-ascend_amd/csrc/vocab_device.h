@@ -113,18 +113,6 @@ __device__ __forceinline__ Vec16 pack(const float* x) {
   return v;
 }
 
-// Eight consecutive elements of type T as floats.
-template <typename T>
-__device__ __forceinline__ void load8(const typename T::raw* p, float (&x)[8]) {
-  unpack<T>(load16(p), x);
-  if constexpr (kElems<T> == 4) unpack<T>(load16(p + 4), x + 4);
-}
-template <typename T>
-__device__ __forceinline__ void store8(typename T::raw* p, const float (&x)[8]) {
-  store16(p, pack<T>(x));
-  if constexpr (kElems<T> == 4) store16(p + 4, pack<T>(x + 4));
-}
-
 __device__ __forceinline__ int lane_id() { return static_cast<int>(threadIdx.x) & (kWave - 1); }
 
 // The value of the lane whose number differs in bit J (1, 2, 4, 8, 16 or 32), without LDS.
