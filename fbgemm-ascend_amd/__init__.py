@@ -50,7 +50,8 @@ BLOCK_BUCKETIZE_SCHEMA = (
     "Tensor? total_num_blocks=None) -> (Tensor, Tensor, Tensor?, Tensor?, Tensor?)"
 )
 
-# The operators over a vocabulary table and its logits (no counterpart in the reference)
+# The operators over a vocabulary table and its logits (no counterpart in the reference); a
+# padding_idx below 0 is none
 VOCAB_SCHEMAS = (
     "token_embedding(Tensor weight, Tensor token_ids, float scale=1.0, ScalarType? out_dtype=None) -> Tensor",
     "token_embedding_grad(Tensor grad_output, Tensor token_ids, int num_rows, float scale=1.0, "

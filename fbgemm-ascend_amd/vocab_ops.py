@@ -9,7 +9,10 @@
 
 HIP tensors only; calls are asynchronous on the current stream.  float32, float16 and
 bfloat16; sums and softmax statistics are in 32 bits.  A token outside the table or the
-vocabulary contributes nothing.  The same operators are registered as torch.ops.tbe.*.
+vocabulary contributes nothing.  Differentiable ones have a backward pass of first order; forward
+mode raises.  The same kernels are registered as torch.ops.tbe.*, for HIP tensors alone: those
+are not differentiable (their results do not require a gradient) and have no fake kernel for
+tracing.
 """
 from __future__ import annotations
 
@@ -53,7 +56,8 @@ def token_embedding(weight: torch.Tensor, token_ids: torch.Tensor, scale: float 
     """scale * weight[token_ids], in out_dtype (default: the weight's).
 
     token_ids: int32 or int64, any shape; a token outside the table gives a row of zeros.
-    padding_idx: a token whose row gets no gradient (it is looked up like any other)."""
+    padding_idx: a token whose row gets no gradient (it is looked up like any other).  None or
+    a number below 0 is no token: it does not count from the table's end."""
     pad = _NO_PADDING if padding_idx is None else padding_idx
     if _tracks(weight):
         return _TokenEmbeddingFn.apply(weight, token_ids, scale, pad, out_dtype)
@@ -63,7 +67,8 @@ def token_embedding(weight: torch.Tensor, token_ids: torch.Tensor, scale: float 
 def token_embedding_grad(grad_output: torch.Tensor, token_ids: torch.Tensor, num_rows: int, scale: float = 1.0,
                          padding_idx: Optional[int] = None,
                          grad_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """The gradient [num_rows, width] of the table, from that of token_embedding's result."""
+    """The gradient [num_rows, width] of the table, from that of token_embedding's result
+    (padding_idx as there)."""
     return _ext.token_embedding_grad(grad_output, token_ids, num_rows, scale,
                                      _NO_PADDING if padding_idx is None else padding_idx, grad_dtype)
 
