@@ -1238,9 +1238,14 @@ extern "C" int tbe_topk_distill_step(const TbeTopkDistillArgs* a, void* hip_stre
   if (!a->loss || !a->grad_logits) return fail(TBE_ERR_INVALID_ARG, "null pointer argument");
   const hipStream_t stream = static_cast<hipStream_t>(hip_stream);
   DistillParams p = distill_params(a);
-  // Few long rows: one work-group a row leaves the GPU idle, two passes over parts of rows do not
-  // (rows of 256 KiB, two passes / one: 16 rows 16 / 23 us, 64 19 / 23, 100 25 / 23).
-  if (a->num_rows < 96 && a->vocab * (a->logits_dtype == TBE_TY_FP32 ? 4 : 2) > (128 << 10)) {
+  // Few long rows: one work-group a row leaves the GPU idle, two passes over parts of rows do not.
+  // How many rows are few goes with their tokens, whatever the type.  us, two passes / one, bf16 and fp32:
+  //   73728 tokens     8 rows 14.4 / 14.2, 14.1 / 15.3    40 15.8 / 14.8, 18.0 / 15.9
+  //   98304           32 15.2 / 16.3, 18.3 / 18.9         64 18.3 / 16.5, 24.1 / 20.5
+  //   131072          48 18.2 / 20.0, 23.9 / 24.7         80 24.6 / 20.4, 32.4 / 28.8
+  //   262144          96 39.4 / 40.5, 61.0 / 68.8        144 51.1 / 46.6, 84.3 / 83.4
+  //   524288         144 90.3 / 94.8, 164 / 179          192 112 / 107, 217 / 207
+  if (a->vocab >= 81920 && a->num_rows <= std::min<int64_t>(160, a->vocab / 2560)) {
     const int rc = distill_loss(a, p, stream);
     return rc != TBE_OK ? rc : distill_grad(a, p, stream);
   }
