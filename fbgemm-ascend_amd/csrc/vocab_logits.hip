@@ -1018,12 +1018,18 @@ struct RowPlan {
 // That launch pays for shorter rows only with a top list, whose instructions bound the pass, and few rows
 // (fp32, one work-group of 1024 / parts): top 20 1 x 50000 15.0 / 11.7, 24 x 32768 11.8 / 11.1, 128 x 40000 13.7
 // / 14.5; no list 24 x 32768 6.9 / 9.9, 24 x 100003 fp16 10.9 / 9.7.
-// A few long rows more than the 256 CUs are quartered too if lists are asked for: else some CUs have two rows
-// and most one.  Top 64, one part of 512 / four of 256: 260 x 131072 bf16 36.6 / 31.5, 300 x 100003 fp32 39.9 /
-// 35.2; but 230 rows, one to a CU, 24.7 / 26.0 (top 5), 400 39.8 / 43.4, 300 x 32768 14.7 / 16.5, and 300 x
-// 100003 fp16 without lists 16.8 / 18.4.
+// Up to 320 long rows, which as quarters of 256 threads are 1280 work-groups, the 5 that every CU holds at once,
+// are quartered too if lists are asked for: else a CU has one long row or two.  One part of 512 threads / four of
+// 256, the two sides of each edge (no list, 300 x 100003 fp16: 16.8 / 18.4):
+//   bf16, top 5, 300 rows   65536 tokens 22.1 / 21.4   81920 25.1 / 25.9    98304 28.1 / 26.0   131072 33.8 / 29.6
+//         131072 tokens     225 rows 26.6 / 26.3       256 27.1 / 26.6      320 34.1 / 29.8     328 34.1 / 35.3
+//         98304 tokens      225 rows 22.2 / 23.1       256 22.4 / 23.3      257 26.2 / 24.9     320 28.3 / 26.3
+//   fp32, top 5, 300 rows   49152 tokens 21.8 / 21.9   65536 26.1 / 24.9    100003, top 64 39.9 / 35.2
+//         65536 tokens      225 rows 22.5 / 22.2       320 26.2 / 25.8      328 26.4 / 27.5     384 27.3 / 30.1
+// Lists of 64 gain more: 225 x 131072 bf16 32.8 / 30.1, fp32 41.4 / 36.3.
 RowPlan row_plan(int64_t rows, int64_t vocab, int32_t dtype, bool lists) {
-  if (lists && rows > 256 && rows <= 320 && vocab >= 98304) return {4, 256};
+  const int64_t quartered = dtype == TBE_TY_FP32 ? 65536 : rows > 256 ? 98304 : 131072;
+  if (lists && rows >= 224 && rows <= 320 && vocab >= quartered) return {4, 256};
   if (rows >= 512) return {1, 256};
   if (rows >= 224) return {1, 512};
   const int64_t one_step = (32 << 10) / (dtype == TBE_TY_FP32 ? 4 : 2);
