@@ -507,8 +507,8 @@ __device__ __forceinline__ void finish_row(const LogprobsParams& p, const Given&
 }
 
 // A work-group per row, or per part of a row (then logprobs_join_kernel finishes the row).  One pass
-// over the logits, bound by HBM without a top list (2048 rows of 131072 bf16 98 us, 5.5 TB/s) and by
-// its instructions with one (top 20 123 us, top 64 131 us).
+// over the logits, bound by HBM without a top list (2048 rows of 131072 bf16 95 us, 5.6 TB/s) and by
+// its instructions with one (top 20 117 us, top 64 128 us).
 template <int kSize, typename T, bool kTop>
 __global__ __launch_bounds__(kSize) void logprobs_kernel(LogprobsParams p, Parts parts, int64_t first) {
   __shared__ GroupShared<kSize> sh;
