@@ -824,12 +824,12 @@ __device__ __forceinline__ float row_weight(const DistillParams& p, int64_t i) {
   return p.weights ? p.weights[i] : 1.f;
 }
 
-// A thread's term of sum q (log q - log p).
-__device__ __forceinline__ float loss_term(const Entry& t, const Stats& st, float log_s, float inv_t) {
+// A thread's term of T sum q (log q - log p): log p, a difference of logits by T, may leave the range
+// where T log p does not (listed tokens that a low value masks, low temperatures).
+__device__ __forceinline__ float loss_term(const Entry& t, const Stats& st, float log_s, float temperature) {
   if (t.id < 0 || t.q == 0.f) return 0.f;
-  // q before 1 / T: of a logit of the type's lowest value the quotient may leave the range
   const float d = st.empty() ? -INFINITY : t.x - st.m;
-  return t.q * (t.log_q + log_s) - t.q * d * inv_t;
+  return t.q * fmaf(t.log_q + log_s, temperature, -d);
 }
 
 __device__ __forceinline__ void store_row(const DistillParams& p, int64_t i, float loss, float m, float s) {
@@ -843,8 +843,8 @@ template <int kSize>
 __device__ __forceinline__ void finish_loss(const DistillParams& p, int64_t i, float weight, const Entry& t,
                                             const Stats& st, GroupShared<kSize>& sh) {
   const float log_s = st.log_s(p.c);
-  const float loss = group_sum(loss_term(t, st, log_s, p.inv_t), sh);
-  store_row(p, i, weight * (p.t * (p.t * loss)), st.m, st.sum(p.c));
+  const float loss = group_sum(loss_term(t, st, log_s, p.t), sh);
+  store_row(p, i, weight * (p.t * loss), st.m, st.sum(p.c));
 }
 
 // A work-group per row, or per part of a row (then distill_join_kernel finishes the row).
@@ -961,9 +961,9 @@ __global__ __launch_bounds__(kSize) void distill_step_kernel(DistillParams p, in
   row_pass<kSize, T, false, false>(row, held, row.nvec, true, st, none);
   join_group(st, p.c, sh);
   const float m = st.m, log_s = st.log_s(p.c);
-  float loss = loss_term(t, st, log_s, p.inv_t), total = t.q;
+  float loss = loss_term(t, st, log_s, p.t), total = t.q;
   group_sum(loss, total, sh);
-  store_row(p, i, weight * (p.t * (p.t * loss)), m, st.sum(p.c));
+  store_row(p, i, weight * (p.t * loss), m, st.sum(p.c));
   if (st.empty() || total == 0.f) {  // no student or no teacher
     zero_row<kSize>(row, out, range);
     return;
