@@ -83,15 +83,14 @@ struct Scale {
   }
 };
 
-// Running maximum m, s = sum 2^y and t = sum 2^y y over the logits so far, in 32 bits.
-// A NaN among the x leaves m alone and makes s NaN; x of -inf adds nothing.
+// Maximum m, s = sum exp((x - m) / T) and t = sum exp((x - m) / T) y, y = log2(e) (x - m) / T, over the
+// logits so far, in 32 bits.  A NaN among the x leaves m alone and makes s NaN; x of -inf adds nothing.
 struct Stats {
   float m, s, t;
 
   __device__ static Stats none() { return {-INFINITY, 0.f, 0.f}; }
-  // Moves the maximum to nm > m and the sums from scale to scale.
-  __device__ void raise(float nm, const Scale& from, const Scale& to) {
-    const float delta = fmaf(to.off - from.off, to.c, to.M - from.M);  // rests and all
+  // Moves the maximum to nm > m, by which y falls by delta.
+  __device__ void raise(float nm, float delta) {
     const float r = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-delta);
     t = r == 0.f ? 0.f : r * (t - delta * s);
     s *= r;  // 0 * NaN stays NaN
@@ -101,21 +100,17 @@ struct Stats {
   template <int N>
   __device__ void join_lanes(float c) {
     const float most = lanes_max<N>(m);
-    if (most > m) raise(most, Scale(m, c), Scale(most, c));
+    if (most > m) raise(most, (most - m) * c);
     s = lanes_sum<N>(s);
     t = lanes_sum<N>(t);
   }
   __device__ bool empty() const { return m == -INFINITY && s == 0.f; }  // no token is possible
-  // sum exp((x - m) / T) and its logarithm
-  __device__ float sum(float c) const { return empty() ? 0.f : s * __builtin_amdgcn_exp2f(-Scale(m, c).rest); }
-  __device__ float log_s(float c) const {
-    return empty() ? 0.f : (__builtin_amdgcn_logf(s) - Scale(m, c).rest) * kLn2;
-  }
+  __device__ float log_s() const { return empty() ? 0.f : __builtin_amdgcn_logf(s) * kLn2; }
   __device__ float entropy() const { return empty() ? 0.f : (__builtin_amdgcn_logf(s) - t / s) * kLn2; }
 };
 
-// Statistics of the logits that one thread meets, and the scale of their maximum.  The maximum
-// moves seldom after the first vectors: a wave looks whether any lane's does.
+// Statistics of the logits that one thread meets, on the scale of their maximum until settle().  The
+// maximum moves seldom after the first vectors: a wave looks whether any lane's does.
 struct Running : Stats {
   float factor;
   Scale scale;
@@ -126,7 +121,7 @@ struct Running : Stats {
     if (__ballot(top > m) != 0) {
       if (top > m) {
         const Scale to(top, factor);
-        raise(top, scale, to);
+        raise(top, fmaf(to.off - scale.off, factor, to.M - scale.M));  // from scale to scale, rests and all
         scale = to;
       }
       far = __ballot(scale.off != 0.f) != 0;
@@ -147,6 +142,13 @@ struct Running : Stats {
     }
     s += near_s;
     if constexpr (kEnt) t += near_t;
+  }
+  // Takes the scale's rest out, after the last logit.
+  __device__ __forceinline__ void settle() {
+    if (m == -INFINITY) return;
+    const float rest = Scale(m, factor).rest, r = __builtin_amdgcn_exp2f(-rest);
+    t = r * (t - rest * s);
+    s *= r;
   }
 };
 
@@ -360,6 +362,7 @@ __device__ __forceinline__ void row_pass(const Row<T>& row, int32_t v0, int32_t 
     }
   }
   if constexpr (kTop) top.settle(1);
+  st.settle();
 }
 
 template <int kSize>
@@ -489,11 +492,11 @@ __device__ __forceinline__ Given load_given(const LogprobsParams& p, const Row<T
 __device__ __forceinline__ void finish_row(const LogprobsParams& p, const Given& given, int64_t i, const Stats& st,
                                            uint64_t list) {
   const bool empty = st.empty();
-  const float log_s = st.log_s(p.c);
+  const float log_s = st.log_s();
   if (threadIdx.x == 0) {
     p.entropy[i] = st.entropy();
     p.stats[2 * i] = st.m;
-    p.stats[2 * i + 1] = st.sum(p.c);
+    p.stats[2 * i + 1] = st.s;
   }
   if (given.some) {
     const float lp = empty ? -INFINITY : (given.x - st.m) / p.t - log_s;
@@ -842,9 +845,9 @@ __device__ __forceinline__ void store_row(const DistillParams& p, int64_t i, flo
 template <int kSize>
 __device__ __forceinline__ void finish_loss(const DistillParams& p, int64_t i, float weight, const Entry& t,
                                             const Stats& st, GroupShared<kSize>& sh) {
-  const float log_s = st.log_s(p.c);
+  const float log_s = st.log_s();
   const float loss = group_sum(loss_term(t, st, log_s, p.t), sh);
-  store_row(p, i, weight * (p.t * loss), st.m, st.sum(p.c));
+  store_row(p, i, weight * (p.t * loss), st.m, st.s);
 }
 
 // A work-group per row, or per part of a row (then distill_join_kernel finishes the row).
@@ -960,16 +963,16 @@ __global__ __launch_bounds__(kSize) void distill_step_kernel(DistillParams p, in
   const int32_t held = std::min(row.nvec, kSize * kHeld);
   row_pass<kSize, T, false, false>(row, held, row.nvec, true, st, none);
   join_group(st, p.c, sh);
-  const float m = st.m, log_s = st.log_s(p.c);
+  const float m = st.m, log_s = st.log_s();
   float loss = loss_term(t, st, log_s, p.t), total = t.q;
   group_sum(loss, total, sh);
-  store_row(p, i, weight * (p.t * loss), m, st.sum(p.c));
+  store_row(p, i, weight * (p.t * loss), m, st.s);
   if (st.empty() || total == 0.f) {  // no student or no teacher
     zero_row<kSize>(row, out, range);
     return;
   }
   const Scale scale(m, p.c);
-  const float a = wt * total / st.s;  // s is of the same scale
+  const float a = grad_factor(wt * total, scale, st.s);
   auto f = [&](float y) { return a * __builtin_amdgcn_exp2f(y); };
   scale.with([&](auto y) {
 #pragma unroll
